@@ -1,0 +1,53 @@
+"""Rules on the text of the sources, scripts and build files (no GPU, no compiler).
+
+* Device code writes through the vector path only.  A write through the scalar data cache is not coherent with it and needs
+  a write-back of its own before anything else can see it.  Comments and strings count: what is not written about is not
+  copied from there into a kernel.
+"""
+import os
+import re
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+SKIP = {".git", "__pycache__", "_work", "_ref", "build", "gpurun_out"}   # not tracked
+SUFFIXES = (".hip", ".h", ".hpp", ".inc", ".c", ".cpp", ".s", ".S", ".ll", ".py", ".sh", ".go", ".mk", ".cmake")
+
+# Scalar stores, scalar atomics, and the scalar cache's write-back and discard; the names are put together here so that
+# this file itself holds none.  In a string of assembly a name may follow an escape (\n, \t) without a space.
+S = "s_"
+SCALAR_WRITE = re.compile(rf"(?:(?<!\w)|(?<=\\[nt])){S}(?:(?:(?:buffer|scratch)_)?(?:store|atomic)_\w+|dcache_(?:wb|discard)\w*)")
+
+
+def source_files():
+    for top, dirs, names in os.walk(ROOT):
+        dirs[:] = [d for d in dirs if d not in SKIP]
+        for name in names:
+            if name.endswith(SUFFIXES) or name == "Makefile":
+                yield os.path.join(top, name)
+
+
+def scalar_writes(text):
+    return [(i, m.group(0)) for i, line in enumerate(text.splitlines(), 1) for m in SCALAR_WRITE.finditer(line)]
+
+
+def test_no_source_writes_through_the_scalar_cache():
+    files = list(source_files())
+    assert any(f.endswith(".hip") for f in files) and any(f.endswith("Makefile") for f in files)
+    found = []
+    for path in files:
+        with open(path, encoding="utf-8", errors="replace") as f:
+            found += [f"{os.path.relpath(path, ROOT)}:{i}: {what}" for i, what in scalar_writes(f.read())]
+    assert not found, found
+
+
+@pytest.mark.parametrize("tail", ["store_dword", "store_dwordx4", "buffer_store_dwordx2", "scratch_store_dword", "atomic_add",
+                                  "buffer_atomic_cmpswap_x2", "dcache_wb", "dcache_wb_vol", "dcache_discard_x2"])
+def test_the_pattern_sees_every_form(tail):
+    assert scalar_writes(f'asm volatile("{S}{tail} %0, %1, 0x0\\n\\t{S}{tail}");  // and {S}{tail}\n') == [(1, S + tail)] * 3
+
+
+@pytest.mark.parametrize("line", [S + "load_dwordx4 s[0:3], s[4:5], 0x0", S + "dcache_inv", "global_store_dword v0, v1, s[0:1]",
+                                  "buffer_store_dwordx4 v[0:3], v4, s[0:3], 0 offen", "ds_write_b32 v0, v1", "words_store_x"])
+def test_the_pattern_leaves_other_code_alone(line):
+    assert scalar_writes(line) == []
