@@ -3,6 +3,7 @@
 * Device code writes through the vector path only.  A write through the scalar data cache is not coherent with it and needs
   a write-back of its own before anything else can see it.  Comments and strings count: what is not written about is not
   copied from there into a kernel.
+* A variant of the store microbenchmark that its main() does not launch has no figure that can be checked.
 """
 import os
 import re
@@ -51,3 +52,12 @@ def test_the_pattern_sees_every_form(tail):
                                   "buffer_store_dwordx4 v[0:3], v4, s[0:3], 0 offen", "ds_write_b32 v0, v1", "words_store_x"])
 def test_the_pattern_leaves_other_code_alone(line):
     assert scalar_writes(line) == []
+
+
+def test_every_store_variant_of_the_microbenchmark_is_launched():
+    with open(os.path.join(ROOT, "tools", "sst_bench.hip"), encoding="utf-8") as f:
+        kernel, main = f.read().split("int main()")
+    launched = {int(st) for st in re.findall(r"run<(\d+), \d+>\(d, o\)", main)}
+    single = {int(st) for st in re.findall(r"ST == (\d+)", kernel)}
+    assert single == {st for st in launched if st < 10}
+    assert "ST >= 10" in kernel and any(st >= 10 for st in launched)

@@ -48,9 +48,6 @@ __global__ __launch_bounds__(64, 2) void k(const uint8_t *src, uint32_t *out, in
                 for (int j = 0; j < N / 2; ++j) { v4 x = {acc + j, ~acc, acc ^ j, acc}; o4[j * 64 + lane] = x; }
             }
         }
-        if (ST == 6) { const int tr = (t + wg * 5) & 63; ob[(2 * tr) * 64 + lane] = acc; ob[(2 * tr + 1) * 64 + lane] = ~acc; }
-        if (ST == 7) { uint32_t *oc = out + ((size_t)t * 2048 + wg) * 128; oc[lane] = acc; oc[64 + lane] = ~acc; }   // time-major: all waves' tile-t output contiguous
-        if (ST == 8) { const uint32_t h = (wg * 2654435761u) >> 21; uint32_t *oc = out + ((size_t)t * 2048 + h) * 128; oc[lane] = acc; oc[64 + lane] = ~acc; }
     }
     if (ST == 0) out[wg * 64 + lane] = acc;
 }
