@@ -134,7 +134,7 @@ struct K1Geom {
     static constexpr int NPT = HBA / kTileBytes;      // staging tiles that lie in the halo
     // Output words (32 decisions each) a lane keeps in registers between flushes.  Mixing a trickle of writes
     // into the saturated read stream costs far more than the bytes (tools/sst_bench.hip: 64 MiB written per
-    // tile step +35 % kernel time, the same bytes in a few chip-wide bursts +3 %), so the bits are held in
+    // tile step +40 % kernel time, the same bytes in one chip-wide burst +9 %), so the bits are held in
     // whatever VGPRs the csum rings leave free (256 per lane at 2 waves per SIMD) and written in bursts.
 #ifdef AMR_K1_NW
     static constexpr int NW = AMR_K1_NW;

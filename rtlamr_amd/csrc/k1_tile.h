@@ -62,7 +62,7 @@ __device__ unsigned long long k1t_timeline[kK1TLaunches][kK1TWgs][3];
 // NLC    finished output chunks (4 words per lane = 1 KiB per wave) parked in LDS between store bursts, on top of the
 //        NW words kept in registers and the 4-word staging chunk: a burst is 4 * (NLC + 1) + NW words per lane.
 //        Output stores mixed into the read stream cost far more than their bytes, and the cost goes with the number
-//        of bursts (tools/sst_bench.hip: 64 MiB in 8 / 4 / 2 / 1 chip-wide bursts: +30 / +23 / +15 / +8 %).
+//        of bursts (tools/sst_bench.hip: 64 MiB in 8 / 4 / 2 / 1 chip-wide bursts: +31 / +26 / +17 / +9 %).
 // PRIO   the two waves of a SIMD do not share it fairly: the arbiter prefers the older wave, which then finishes ~9 %
 //        earlier and leaves the younger one alone (no latency hiding, half the memory parallelism) for the rest of the
 //        launch.  1: the wave in the odd hardware slot runs at priority 1 throughout; 2 / 3 / 4: the two waves swap
