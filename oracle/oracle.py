@@ -40,7 +40,7 @@ def build(force: bool = False) -> str:
     """Compile liboracle.so with the committed Makefile (gcc, seconds)."""
     srcs = [os.path.join(_HERE, f) for f in ("decode_oracle.c", "synth_gen.c", "Makefile")]
     if force or not os.path.exists(_SO) or os.path.getmtime(_SO) < max(os.path.getmtime(f) for f in srcs):
-        subprocess.check_call(["make", "-C", _HERE, "-s", "liboracle.so"])
+        subprocess.check_call(["make", "-C", _HERE, "-s", "liboracle.so"] + (["-B"] if force else []))
     return _SO
 
 
