@@ -4,6 +4,7 @@
   a write-back of its own before anything else can see it.  Comments and strings count: what is not written about is not
   copied from there into a kernel.
 * A variant of the store microbenchmark that its main() does not launch has no figure that can be checked.
+* No packed FP32 arithmetic: neither written by hand nor left to the compiler.
 """
 import os
 import re
@@ -61,3 +62,20 @@ def test_every_store_variant_of_the_microbenchmark_is_launched():
     single = {int(st) for st in re.findall(r"ST == (\d+)", kernel)}
     assert single == {st for st in launched if st < 10}
     assert "ST >= 10" in kernel and any(st >= 10 for st in launched)
+
+
+PACKED_OFF = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+
+
+def test_device_code_is_compiled_without_packed_fp32():
+    """hipcc -O3 forms packed float operations from scalar code by itself; every compile line of device code rules them out."""
+    lines = []
+    for path in source_files():
+        if os.path.dirname(path) == os.path.join(ROOT, "tests"):
+            continue                                     # host programs only
+        with open(path, encoding="utf-8", errors="replace") as f:
+            lines += [(path, line) for line in f if "--offload-arch" in line and "-shared" not in line]
+    with open(os.path.join(ROOT, "tools", "README.md"), encoding="utf-8") as f:
+        lines += [(f.name, line) for line in f if "--offload-arch" in line]
+    assert any(path.endswith("csrc/Makefile") for path, _ in lines)
+    assert [(path, line) for path, line in lines if PACKED_OFF not in line] == []

@@ -3,7 +3,7 @@
 # print resource usage of matching kernels; the kernel ISA goes to /tmp/k1asm/<n>.s
 set -e
 mkdir -p /tmp/k1asm && cd /tmp/k1asm
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC ${EXTRA_FLAGS} -I/root/repo/include -I/root/repo/rtlamr_amd/csrc -save-temps -c /root/repo/rtlamr_amd/csrc/${2:-amr_pipeline.hip} -o /tmp/k1asm/a.o
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off -fPIC ${EXTRA_FLAGS} -I/root/repo/include -I/root/repo/rtlamr_amd/csrc -save-temps -c /root/repo/rtlamr_amd/csrc/${2:-amr_pipeline.hip} -o /tmp/k1asm/a.o
 S=amrdemod-hip-amdgcn-amd-amdhsa-gfx950.s
 python3 - "$1" <<'PY'
 import re,sys

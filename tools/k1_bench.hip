@@ -1,7 +1,7 @@
 // Developer harness (not product code): times K1 alone, without Python/torch, so that many kernel variants can be
 // compared in one short GPU session.  Build one binary per variant, e.g.
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fno-slp-vectorize -Irtlamr_amd/csrc -Iinclude \
-//         -DK1B_CL=72 [-DAMR_K1T_SCHED=1 ...] -o build/k1b_<tag> tools/k1_bench.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -ffp-contract=off \
+//         -fno-slp-vectorize -Irtlamr_amd/csrc -Iinclude -DK1B_CL=72 [-DAMR_K1T_SCHED=1 ...] -o build/k1b_<tag> tools/k1_bench.hip
 // usage: k1b [variants: comma list of names, or "all"] [n_blocks] [reps] [input: 0 noise, 1 uniform bytes] [n_allocs] [block_size] [spin-up launches]
 // All variants live in one binary and run round-robin on the same buffers (K1's time depends on the process's
 // allocation and on the shader clock's ramp-up, so only same-process, interleaved comparisons mean anything).

@@ -1,7 +1,8 @@
 // K2 harness: k2_search_walk<SL, SET> alone on a random bitstream, with the per-wave phase stamps of AMR_K2W_DBG
 // (developer tool, not product code).  Geometry: scm at chip length 72 by default (rows of 128 words), or "idm" / "all"
 // (rows of 256 words).
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -DAMR_K2W_DBG=1 -DAMR_K2R_LPR2=1 -Irtlamr_amd/csrc -Iinclude -o build/k2b tools/k2_bench.hip
+//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -DAMR_K2W_DBG=1 \
+//         -DAMR_K2R_LPR2=1 -Irtlamr_amd/csrc -Iinclude -o build/k2b tools/k2_bench.hip
 // usage: k2b [scm|idm|all] [n_tiles incl. the history tile] [reps] [cold]
 // "scm" also runs k2_search_row<144, 0, 128> (k2_row.h) on the same bitstream and compares counts and staging with the walk;
 // cold: a 1 GiB buffer is streamed through the chip in front of every launch (what K1 does to the caches in the product)
