@@ -79,3 +79,11 @@ def test_device_code_is_compiled_without_packed_fp32():
         lines += [(f.name, line) for line in f if "--offload-arch" in line]
     assert any(path.endswith("csrc/Makefile") for path, _ in lines)
     assert [(path, line) for path, line in lines if PACKED_OFF not in line] == []
+
+
+def test_no_packed_fp32_by_hand():
+    packed = re.compile(r"\bv_pk_(?:add|mul|fma)_f32\b")
+    for path in source_files():
+        if path.endswith((".hip", ".h", ".inc")):
+            with open(path, encoding="utf-8", errors="replace") as f:
+                assert not packed.search(f.read()), path

@@ -10,7 +10,6 @@ __global__ void k(float *out, int iters, uint64_t *cyc)
     for (int i = threadIdx.x; i < 1024; i += blockDim.x) lut[i] = i;
     __syncthreads();
     float a0 = threadIdx.x, a1 = 1, a2 = 2, a3 = 3, a4 = 4, a5 = 5, a6 = 6, a7 = 7, b = 1.5f;
-    float2 p0 = {1, 2}, p1 = {3, 4}, p2 = {5, 6}, p3 = {7, 8}, pb = {1.5f, 2.5f};
     uint32_t u0 = threadIdx.x, u1 = 77;
     uint32_t addr = (threadIdx.x & 31) * 4;
     uint64_t t0 = __builtin_readcyclecounter();
@@ -20,9 +19,6 @@ __global__ void k(float *out, int iters, uint64_t *cyc)
                          : "+v"(a0), "+v"(a1), "+v"(a2), "+v"(a3), "+v"(a4), "+v"(a5), "+v"(a6), "+v"(a7) : "v"(b));
         } else if (MODE == 1) {  // 32 dependent v_add_f32
             asm volatile(REP8("v_add_f32 %0, %0, %1\n v_add_f32 %0, %0, %1\n v_add_f32 %0, %0, %1\n v_add_f32 %0, %0, %1\n") : "+v"(a0) : "v"(b));
-        } else if (MODE == 2) {  // 32 independent v_pk_add_f32 (4 chains)
-            asm volatile(REP8("v_pk_add_f32 %0, %0, %4\n v_pk_add_f32 %1, %1, %4\n v_pk_add_f32 %2, %2, %4\n v_pk_add_f32 %3, %3, %4\n")
-                         : "+v"(p0), "+v"(p1), "+v"(p2), "+v"(p3) : "v"(pb));
         } else if (MODE == 3) {  // 2-chain dependent v_add (distance 2)
             asm volatile(REP8("v_add_f32 %0, %0, %2\n v_add_f32 %1, %1, %2\n v_add_f32 %0, %0, %2\n v_add_f32 %1, %1, %2\n") : "+v"(a0), "+v"(a1) : "v"(b));
         } else if (MODE == 4) {  // K1-like dependent group: add, sub, sub, alignbit
@@ -46,7 +42,7 @@ __global__ void k(float *out, int iters, uint64_t *cyc)
         }
     }
     uint64_t t1 = __builtin_readcyclecounter();
-    out[blockIdx.x * blockDim.x + threadIdx.x] = a0 + a1 + a2 + a3 + a4 + a5 + a6 + a7 + p0.x + p1.y + p2.x + p3.y + u0;
+    out[blockIdx.x * blockDim.x + threadIdx.x] = a0 + a1 + a2 + a3 + a4 + a5 + a6 + a7 + u0;
     if (threadIdx.x == 0 && blockIdx.x == 0) *cyc = t1 - t0;
 }
 template <int MODE>
@@ -73,7 +69,6 @@ int main()
 {
     run<0>("v_add_f32 indep x32", 32);
     run<1>("v_add_f32 dependent x32", 32);
-    run<2>("v_pk_add_f32 indep x32", 32);
     run<3>("v_add_f32 2-chain x32", 32);
     run<4>("add,sub,sub,alignbit dep x32", 32);
     run<5>("ds_read_b32 x16 + wait", 16);
