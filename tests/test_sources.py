@@ -12,7 +12,7 @@ import re
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-SKIP = {".git", "__pycache__", "_work", "_ref", "build", "gpurun_out"}   # not tracked
+TREES = ("rtlamr_amd", "include", "tests", "tools", "oracle", "go", "docs", "profiles")   # and the files at the top
 SUFFIXES = (".hip", ".h", ".hpp", ".inc", ".c", ".cpp", ".s", ".S", ".ll", ".py", ".sh", ".go", ".mk", ".cmake")
 
 # Scalar stores, scalar atomics, and the scalar cache's write-back and discard; the names are put together here so that
@@ -22,8 +22,10 @@ SCALAR_WRITE = re.compile(rf"(?:(?<!\w)|(?<=\\[nt])){S}(?:(?:(?:buffer|scratch)_
 
 
 def source_files():
-    for top, dirs, names in os.walk(ROOT):
-        dirs[:] = [d for d in dirs if d not in SKIP]
+    walks = [(ROOT, [], os.listdir(ROOT))]
+    for tree in TREES:
+        walks += os.walk(os.path.join(ROOT, tree))
+    for top, _, names in walks:
         for name in names:
             if name.endswith(SUFFIXES) or name == "Makefile":
                 yield os.path.join(top, name)
